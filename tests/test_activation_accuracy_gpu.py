@@ -1,0 +1,87 @@
+"""The activations of checkpointed tensors in fp32 to a few units of its last bit, and 16-bit results down to their type's least number.
+
+Tolerances count half steps of fp32 (UNIT, relative to the value).  The hardware's power of two and reciprocal are off by one step, two
+UNIT, the sums and products of a formula by one UNIT each, and a result below the normal numbers by half the least number."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from helpers import copy_numpy_to_gpu
+from row_operations import FORMATS, UNIT, decode, download, rounding, upload, value_and_slope, within
+from thor_amd import physical as ph
+from thor_amd.dtypes import DataType
+
+pytestmark = pytest.mark.gpu
+LEAST = 2.0**-149
+SWISH, GELU = ph.ActivationKind.swish, ph.ActivationKind.gelu
+
+
+@pytest.fixture(scope="module")
+def stream(gpu):
+    return ph.Stream(0)
+
+
+def grid():
+    """From beyond the deepest tail to beyond where both functions are x, dense where they bend; rows end inside a chunk."""
+    x = np.concatenate([np.linspace(-112, 112, 40001), np.linspace(-15, 15, 60001), -np.logspace(-30, 2, 3000), [0.0, -0.0, -3e38, 3e38]])
+    return np.pad(x, (0, -len(x) % 259)).astype(np.float32).reshape(-1, 259)
+
+
+def forward(kind, x, dtype, stream):
+    tx, x64 = upload(x, dtype, stream)
+    plan = ph.CheckpointedActivation(kind, DataType.int8).stamp(tx, stream)
+    plan.run()
+    return download(plan.get_output_tensor(), stream), x64
+
+
+def backward(kind, dtype, stream):
+    """(dx, dz, x) for an error and a multiplier of ones, at every int8 code of scales from 2^-30 to 1."""
+    codes = np.concatenate([[-127], np.arange(-127, 128), [1, -1, 127]]).astype(np.int8)[None].repeat(400, 0)
+    scales = np.concatenate([np.linspace(0.002, 0.9, 390), 2.0**-np.arange(3.0, 33.0, 3.0)]).astype(np.float32)[:, None].repeat(3, 1)
+    kept = ph.ActivationCheckpoint(copy_numpy_to_gpu(codes, stream, DataType.int8), copy_numpy_to_gpu(scales, stream, DataType.fp32))
+    one = ph.ActivationCheckpoint(copy_numpy_to_gpu(np.ones_like(codes), stream, DataType.int8), copy_numpy_to_gpu(np.ones_like(scales), stream, DataType.fp32))
+    tdy, _ = upload(np.ones(codes.shape), dtype, stream)
+    plan = ph.CheckpointedActivationBackward(kind).stamp(tdy, kept, stream, multiplier_checkpoint=one)
+    plan.run()
+    return download(plan.get_input_gradient_tensor(), stream), download(plan.get_multiplier_gradient_tensor(), stream), decode(codes, scales, DataType.int8).astype(np.float64)
+
+
+def terms(kind, x):
+    """The two terms of the slope, each as a magnitude: s and |x s (1 - s)|, or Phi and |x| phi."""
+    if kind == SWISH:
+        s, rest = np.exp(-np.logaddexp(0, -x)), np.exp(-np.logaddexp(0, x))
+        return s + np.abs(x) * s * rest
+    f, slope, _, _ = value_and_slope(kind, x)
+    phi = np.where(x == 0, 0.5, f / np.where(x == 0, 1.0, x))
+    return phi + np.abs(slope - phi)
+
+
+def test_swish_in_fp32(stream):
+    """x s: the power 2, its argument's last rounding 0.2, e r 1, 1 + e 1, the reciprocal 2, the product with x 1: 7.2 UNIT, taken as 8.
+    The slope s + x s (1 - s): 6.2 of s, and 13.4 and a rounding of the other term: 16 of both."""
+    got, x = forward(SWISH, grid(), DataType.fp32, stream)
+    f = value_and_slope(SWISH, x)[0]
+    within(got, f, 8 * UNIT * np.abs(f) + LEAST, "f")
+    dx, dz, x = backward(SWISH, DataType.fp32, stream)
+    f, slope, _, _ = value_and_slope(SWISH, x)
+    within(dx, slope, 16 * UNIT * terms(SWISH, x) + LEAST, "slope")
+    within(dz, f, 8 * UNIT * np.abs(f) + LEAST, "f backward")
+
+
+@pytest.mark.parametrize("kind", [SWISH], ids=lambda k: k.name)
+@pytest.mark.parametrize("dtype", [DataType.bf16, DataType.fp16], ids=lambda d: d.name)
+def test_results_of_16_bits_down_to_the_least(stream, dtype, kind):
+    """One rounding to the type, and before it what fp32 exponents of up to 190 lose: half of 2^-16 times ln 2 for the exponent's own
+    rounding, twice for gelu's square, 1.1e-5, and the units of the formula: 2e-5 in all."""
+    got, x = forward(kind, np.clip(grid(), -60000, 60000), dtype, stream)
+    f = value_and_slope(kind, x)[0]
+    off = 2e-5 * np.abs(f)
+    within(got, f, off + rounding(np.abs(f) + off, dtype), "f")
+    dx, dz, x = backward(kind, dtype, stream)
+    f, slope, _, _ = value_and_slope(kind, x)
+    off = 2e-5 * terms(kind, x)
+    within(dx, slope, off + rounding(np.abs(slope) + off, dtype), "slope")
+    off = 2e-5 * np.abs(f)
+    within(dz, f, off + rounding(np.abs(f) + off, dtype), "f backward")
+

@@ -87,56 +87,90 @@ __device__ __forceinline__ float tailFactor(float a) {
     p = __builtin_fmaf(p, t, 0.1196320071032971f);
     return p * t;
 }
-// exp(-x^2 / 2) and sigmoid(x), through the hardware's power of two and reciprocal (one unit each).
+
+// exp(-x^2 / 2) through the hardware's power of two.
 __device__ __forceinline__ float bell(float x) { return __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f); }
-__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f)); }
 
-// f(x).
-template <int KIND>
-__device__ __forceinline__ float activate(float x) {
-    if constexpr (KIND == THORHIP_RELU) {
-        return x < 0.0f ? 0.0f : x;  // a NaN stays one
-    } else if constexpr (KIND == THORHIP_GELU) {
-        const float below = tailFactor(__builtin_fabsf(x)) * bell(x);
-        return x * (x < 0.0f ? below : 1.0f - below);
-    } else {
-        return x * sigmoid(x);
+// 2^32 sigmoid(x) for results of 16 bits, through the hardware's power of two and reciprocal.  Those know no numbers below 2^-126, which a
+// bf16 result can be made of: 2^32 brings everything that its type can hold into their range.  The exponent is rounded to fp32, which
+// costs |x| units of 2^-24 in the tail, 7e-6 at most, and up to 7e-7 near zero; a result rounds by 2^-9 or 2^-12.
+__device__ __forceinline__ float sigmoidTimes2To32(float x) {
+    return __builtin_amdgcn_rcpf(0x1p-32f + __builtin_amdgcn_exp2f(__builtin_fmaf(x, -1.4426950408889634f, -32.0f)));
+}
+
+// Results of fp32: a power of two as factor * 2^exponent, of an argument hi + lo with |lo| far below one, so that its rounding does not
+// grow with it and no result is below the numbers that the hardware's power knows.
+struct Power {
+    float factor;
+    int exponent;
+    __device__ __forceinline__ float times(float x) const { return __builtin_ldexpf(x, exponent); }  // 2^exponent x
+    __device__ __forceinline__ float value() const { return times(factor); }
+};
+__device__ __forceinline__ Power powerOfTwo(float hi, float lo) {
+#pragma clang fp contract(off)  // a fused hi - whole would bring what lo holds a second time
+    const float whole = __builtin_rintf(hi);
+    return {__builtin_amdgcn_exp2f(hi - whole + lo), (int)whole};
+}
+// exp(-a) for a in [0, 200]: log2(e) in two parts, and what the products lose.
+__device__ __forceinline__ Power exponential(float a) {
+#pragma clang fp contract(off)
+    const float hi = a * -1.44269502f;
+    return powerOfTwo(hi, __builtin_fmaf(a, -1.92596303e-8f, __builtin_fmaf(a, -1.44269502f, -hi)));
+}
+
+// What the activations are made of at one x: f(x) of a finite x, f(x) of any x, and f'(x).
+template <typename T, int KIND>
+struct Activated;
+
+template <typename T>
+struct Activated<T, THORHIP_RELU> {
+    float x;
+    __device__ __forceinline__ explicit Activated(float x) : x(x) {}
+    __device__ __forceinline__ float finite() const { return any(); }
+    __device__ __forceinline__ float any() const { return x < 0.0f ? 0.0f : x; }  // a NaN stays one
+    __device__ __forceinline__ float slope() const { return x > 0.0f ? 1.0f : x != x ? x : 0.0f; }
+};
+
+// 16 bits: f = x s, f' = s + f (1 - s).
+template <typename T>
+struct Activated<T, THORHIP_SWISH> {
+    float x, s;
+    __device__ __forceinline__ explicit Activated(float x) : x(x), s(sigmoidTimes2To32(x) * 0x1p-32f) {}
+    __device__ __forceinline__ float finite() const { return any(); }
+    __device__ __forceinline__ float any() const { return x * s; }
+    __device__ __forceinline__ float slope() const { return __builtin_fmaf(any(), 1.0f - s, s); }
+};
+// fp32: with e = exp(-|x|) and r = 1 / (1 + e) the sigmoid is e r below zero and r above, and one less it is the other of the two.
+template <>
+struct Activated<float, THORHIP_SWISH> {
+    float x, within, s, rest;  // within: x where the product with s, which is without its power of two, is finite
+    int exponent;
+    __device__ __forceinline__ explicit Activated(float x) : x(x), within(x < -200.0f ? -200.0f : x) {
+        const Power e = exponential(__builtin_amdgcn_fmed3f(__builtin_fabsf(x), 0.0f, 200.0f));
+        const float value = e.value(), r = __builtin_amdgcn_rcpf(1.0f + value);
+        s = x < 0.0f ? e.factor * r : r;
+        rest = x < 0.0f ? r : value * r;
+        exponent = x < 0.0f ? e.exponent : 0;
     }
-}
+    __device__ __forceinline__ float finite() const { return __builtin_ldexpf(within * s, exponent); }
+    __device__ __forceinline__ float any() const { return x * __builtin_ldexpf(s, exponent); }
+    __device__ __forceinline__ float slope() const { return __builtin_ldexpf(__builtin_fmaf(within * s, rest, s), exponent); }
+};
 
-// The same of a finite x: gelu is max(x, 0) - |x| Phi(-|x|), two instructions less than by cases (bf16 16384 x 8192
-// forward 126 -> 121 us: the one kernel here that the vector units bound).
-template <int KIND>
-__device__ __forceinline__ float activateFinite(float x) {
-    if constexpr (KIND != THORHIP_GELU) return activate<KIND>(x);
-    const float a = __builtin_fabsf(x);
-    return __builtin_fmaf(-a, tailFactor(a) * bell(x), __builtin_fmaxf(x, 0.0f));
-}
-
-// gelu's Phi(x) and its slope Phi + x phi: exp(-x^2 / 2) (H(|x|) - |x| / sqrt(2 pi)) below zero, and that from one above.
-__device__ __forceinline__ void phiAndSlope(float x, float& phi, float& slope) {
-    const float a = __builtin_fabsf(x), h = tailFactor(a), e = bell(x);
-    const float below = h * e, slopeBelow = e * __builtin_fmaf(a, -0.39894228040143268f, h);
-    phi = x < 0.0f ? below : 1.0f - below;
-    slope = x < 0.0f ? slopeBelow : 1.0f - slopeBelow;
-}
-
-// f(x) and f'(x).
-template <int KIND>
-__device__ __forceinline__ void activateWithSlope(float x, float& f, float& slope) {
-    if constexpr (KIND == THORHIP_RELU) {
-        f = x < 0.0f ? 0.0f : x;
-        slope = x > 0.0f ? 1.0f : x != x ? x : 0.0f;
-    } else if constexpr (KIND == THORHIP_GELU) {
-        float phi;
-        phiAndSlope(x, phi, slope);
-        f = x * phi;
-    } else {
-        const float s = sigmoid(x);
-        f = x * s;
-        slope = __builtin_fmaf(f, 1.0f - s, s);
+// f = max(x, 0) - |x| Phi(-|x|), two instructions less than by cases (bf16 16384 x 8192 forward 126 -> 121 us: the one kernel
+// here that the vector units bound); f' = exp(-x^2 / 2) (H(|x|) - |x| / sqrt(2 pi)) below zero, and that from one above.
+template <typename T>
+struct Activated<T, THORHIP_GELU> {
+    float x, h, e;
+    __device__ __forceinline__ explicit Activated(float x) : x(x), h(tailFactor(__builtin_fabsf(x))), e(bell(x)) {}
+    __device__ __forceinline__ float finite() const { return __builtin_fmaf(-__builtin_fabsf(x), h * e, __builtin_fmaxf(x, 0.0f)); }
+    __device__ __forceinline__ float any() const { return x * phi(); }
+    __device__ __forceinline__ float phi() const { return x < 0.0f ? h * e : 1.0f - h * e; }
+    __device__ __forceinline__ float slope() const {
+        const float below = e * __builtin_fmaf(__builtin_fabsf(x), -0.39894228040143268f, h);
+        return x < 0.0f ? below : 1.0f - below;
     }
-}
+};
 
 // One operand of the forward pass: its elements, and their codes.
 template <typename T>
@@ -179,14 +213,23 @@ __global__ __launch_bounds__(kThreads) void checkpointedForward(CheckpointedArgs
         if constexpr (KIND != THORHIP_IDENTITY) {
             T* out = rowPointer<T>(a.third, p[u].row, a.innerRows);
             if (p[u].has) {
+                if (scale.times != 0.0f) {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    x[u].v[i] = scale.times != 0.0f ? activateFinite<KIND>(x[u].v[i]) : activate<KIND>(x[u].v[i]);
-                    if constexpr (MULTIPLIED) x[u].v[i] *= z[u].v[i];
+                    for (int i = 0; i < VEC; ++i) x[u].v[i] = Activated<T, KIND>(x[u].v[i]).finite();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) x[u].v[i] = Activated<T, KIND>(x[u].v[i]).any();
+                }
+                if constexpr (MULTIPLIED) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) x[u].v[i] *= z[u].v[i];
                 }
                 storeChunk(out + p[u].column, x[u].v);
             }
-            if (p[u].tail) out[p[u].tailColumn] = narrow<T>(activate<KIND>(x[u].tail) * (MULTIPLIED ? z[u].tail : 1.0f));
+            if (p[u].tail) {
+                const Activated<T, KIND> f(x[u].tail);
+                out[p[u].tailColumn] = narrow<T>((scale.times != 0.0f ? f.finite() : f.any()) * (MULTIPLIED ? z[u].tail : 1.0f));
+            }
         }
     }
 }
@@ -219,10 +262,9 @@ struct GeluTable {
     __device__ static __forceinline__ void fill(float* table) {
         for (u32 i = threadIdx.x; i < kEntries; i += kThreads) {
             const float a = bitsF32((kFirst + i / 2) << 20);
-            float phi, slope;
-            phiAndSlope(i % 2 != 0 ? -a : a, phi, slope);
-            table[i * kWidth] = slope;
-            if constexpr (PAIRS) table[i * kWidth + 1] = phi;
+            const Activated<float, THORHIP_GELU> f(i % 2 != 0 ? -a : a);
+            table[i * kWidth] = f.slope();
+            if constexpr (PAIRS) table[i * kWidth + 1] = f.phi();
         }
     }
     __device__ static __forceinline__ const float* at(const float* table, float x) {
@@ -238,10 +280,9 @@ __device__ __forceinline__ void backward(float dy, float& x, float& z) {
     if constexpr (KIND == THORHIP_IDENTITY) {
         x = finite<T>(x);
     } else {
-        float f, slope;
-        activateWithSlope<KIND>(x, f, slope);
-        x = MULTIPLIED ? dy * z * slope : dy * slope;
-        z = dy * f;
+        const Activated<T, KIND> f(x);
+        x = MULTIPLIED ? dy * z * f.slope() : dy * f.slope();
+        z = dy * f.finite();
     }
 }
 template <bool MULTIPLIED>
