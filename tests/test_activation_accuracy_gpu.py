@@ -7,7 +7,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from helpers import copy_numpy_to_gpu
+from helpers import copy_numpy_to_gpu, from_storage, to_storage
 from row_operations import FORMATS, UNIT, decode, download, rounding, upload, value_and_slope, within
 from thor_amd import physical as ph
 from thor_amd.dtypes import DataType
@@ -28,23 +28,36 @@ def grid():
     return np.pad(x, (0, -len(x) % 259)).astype(np.float32).reshape(-1, 259)
 
 
-def forward(kind, x, dtype, stream):
+def forward(kind, x, dtype, stream, format=DataType.int8):
     tx, x64 = upload(x, dtype, stream)
-    plan = ph.CheckpointedActivation(kind, DataType.int8).stamp(tx, stream)
+    plan = ph.CheckpointedActivation(kind, format).stamp(tx, stream)
     plan.run()
     return download(plan.get_output_tensor(), stream), x64
 
 
-def backward(kind, dtype, stream):
-    """(dx, dz, x) for an error and a multiplier of ones, at every int8 code of scales from 2^-30 to 1."""
-    codes = np.concatenate([[-127], np.arange(-127, 128), [1, -1, 127]]).astype(np.int8)[None].repeat(400, 0)
-    scales = np.concatenate([np.linspace(0.002, 0.9, 390), 2.0**-np.arange(3.0, 33.0, 3.0)]).astype(np.float32)[:, None].repeat(3, 1)
-    kept = ph.ActivationCheckpoint(copy_numpy_to_gpu(codes, stream, DataType.int8), copy_numpy_to_gpu(scales, stream, DataType.fp32))
-    one = ph.ActivationCheckpoint(copy_numpy_to_gpu(np.ones_like(codes), stream, DataType.int8), copy_numpy_to_gpu(np.ones_like(scales), stream, DataType.fp32))
+def backward(kind, dtype, stream, format=DataType.int8):
+    """(dx with and without the multiplier, dz, x) for an error and a multiplier of ones, at every finite code of scales from 2^-30 on: any for int8, powers of two for the
+    others."""
+    if format == DataType.int8:
+        codes = np.concatenate([[-127], np.arange(-127, 128), [1, -1, 127]]).astype(np.int8)
+        scales = np.concatenate([np.linspace(0.002, 0.9, 390), 2.0**-np.arange(3.0, 33.0, 3.0)])
+        one = np.int8(1)
+    else:
+        codes = np.arange(256, dtype=np.uint8)
+        codes = codes[np.isfinite(from_storage(codes, format))]
+        scales = 2.0**np.arange(-30.0, -1.0 if format == DataType.fp8_e4m3 else -9.0)
+        one = to_storage(np.ones(1, np.float32), format)[0]
+    codes = codes[None].repeat(len(scales), 0)
+    scales = scales.astype(np.float32)[:, None].repeat(-(-codes.shape[1] // 128), 1)
+    kept = ph.ActivationCheckpoint(copy_numpy_to_gpu(codes, stream, format), copy_numpy_to_gpu(scales, stream, DataType.fp32))
+    ones = ph.ActivationCheckpoint(copy_numpy_to_gpu(np.full_like(codes, one), stream, format), copy_numpy_to_gpu(np.ones_like(scales), stream, DataType.fp32))
     tdy, _ = upload(np.ones(codes.shape), dtype, stream)
-    plan = ph.CheckpointedActivationBackward(kind).stamp(tdy, kept, stream, multiplier_checkpoint=one)
+    plan = ph.CheckpointedActivationBackward(kind).stamp(tdy, kept, stream, multiplier_checkpoint=ones)
     plan.run()
-    return download(plan.get_input_gradient_tensor(), stream), download(plan.get_multiplier_gradient_tensor(), stream), decode(codes, scales, DataType.int8).astype(np.float64)
+    alone = ph.CheckpointedActivationBackward(kind).stamp(tdy, kept, stream)
+    alone.run()
+    return (np.stack([download(p.get_input_gradient_tensor(), stream) for p in (plan, alone)]), download(plan.get_multiplier_gradient_tensor(), stream),
+            decode(codes, scales, format).astype(np.float64))
 
 
 def terms(kind, x):
@@ -65,11 +78,11 @@ def test_swish_in_fp32(stream):
     within(got, f, 8 * UNIT * np.abs(f) + LEAST, "f")
     dx, dz, x = backward(SWISH, DataType.fp32, stream)
     f, slope, _, _ = value_and_slope(SWISH, x)
-    within(dx, slope, 16 * UNIT * terms(SWISH, x) + LEAST, "slope")
+    within(dx, np.stack([slope, slope]), 16 * UNIT * terms(SWISH, x) + LEAST, "slope")
     within(dz, f, 8 * UNIT * np.abs(f) + LEAST, "f backward")
 
 
-@pytest.mark.parametrize("kind", [SWISH], ids=lambda k: k.name)
+@pytest.mark.parametrize("kind", [SWISH, GELU], ids=lambda k: k.name)
 @pytest.mark.parametrize("dtype", [DataType.bf16, DataType.fp16], ids=lambda d: d.name)
 def test_results_of_16_bits_down_to_the_least(stream, dtype, kind):
     """One rounding to the type, and before it what fp32 exponents of up to 190 lose: half of 2^-16 times ln 2 for the exponent's own
@@ -81,7 +94,20 @@ def test_results_of_16_bits_down_to_the_least(stream, dtype, kind):
     dx, dz, x = backward(kind, dtype, stream)
     f, slope, _, _ = value_and_slope(kind, x)
     off = 2e-5 * terms(kind, x)
-    within(dx, slope, off + rounding(np.abs(slope) + off, dtype), "slope")
+    within(dx, np.stack([slope, slope]), off + rounding(np.abs(slope) + off, dtype), "slope")
     off = 2e-5 * np.abs(f)
     within(dz, f, off + rounding(np.abs(f) + off, dtype), "f backward")
 
+
+@pytest.mark.parametrize("format", FORMATS, ids=lambda f: f.name)
+def test_gelu_in_fp32(stream, format):
+    """x Phi(x): 2.2 the power, 1.3 the reciprocal that the tail's factor follows 2.7 times, 2.6 its polynomial and 1 its last product,
+    two more products: 9.1 UNIT, taken as 10.  Above zero that is what is taken from x.  The slope's two terms have one more product, and
+    above zero the difference from one a rounding: 12 of both."""
+    got, x = forward(GELU, grid(), DataType.fp32, stream, format)
+    f = value_and_slope(GELU, x)[0]
+    within(got, f, 10 * UNIT * np.abs(f) + LEAST, "f")
+    dx, dz, x = backward(GELU, DataType.fp32, stream, format)
+    f, slope, _, _ = value_and_slope(GELU, x)
+    within(dx, np.stack([slope, slope]), 12 * UNIT * terms(GELU, x) + LEAST, "slope")
+    within(dz, f, 10 * UNIT * np.abs(f) + LEAST, "f backward")

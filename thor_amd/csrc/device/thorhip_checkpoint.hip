@@ -73,27 +73,47 @@ __device__ __forceinline__ Place placeOf(const CheckpointedArgs& a, u32 number) 
 }
 
 // Phi(-a) = H(a) exp(-a^2 / 2) for a >= 0.  H falls slowly from 1/2 like 0.4 / a, so a polynomial in t = 1 / (1 + 0.3 a) follows it:
-// t P(t) with the P of degree 7 that is nearest in relative terms on [0, 14.5] (1.7e-7, under three units of fp32; beyond, the
-// exponential is zero).  It shares the exponential with the density, where the library's erfc has one of its own and a division.
+// t P(t) with the P that is nearest in relative terms on [0, 14.5] (beyond, 16-bit results are zero).  It shares the exponential with the
+// density, where the library's erfc has one of its own and a division.
+//
+// fp32: degree 9 (off by 3.5e-9), t from the sum 1 + 0.3 a as it is before its rounding.
+// 16 bits: degree 7 (off by 1.7e-7) at the hardware's reciprocal, some eight units of 2^-24, and H / 2^32 for bellTimes2To32().
+template <typename T>
 __device__ __forceinline__ float tailFactor(float a) {
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.3f, 1.0f));
-    float p = 0.03542373867332211f;
-    p = __builtin_fmaf(p, t, -0.1561584693838267f);
-    p = __builtin_fmaf(p, t, 0.20455683389817478f);
-    p = __builtin_fmaf(p, t, -0.05203407264399261f);
-    p = __builtin_fmaf(p, t, 0.12769180626590437f);
-    p = __builtin_fmaf(p, t, 0.10017593626445624f);
-    p = __builtin_fmaf(p, t, 0.1207121381245411f);
-    p = __builtin_fmaf(p, t, 0.1196320071032971f);
+    const float d = __builtin_fmaf(a, 0.3f, 1.0f);
+    float t = __builtin_amdgcn_rcpf(d);
+    if constexpr (sizeof(T) == 4) {
+        const float lost = __builtin_fmaf(a, 0.3f, 1.0f - d);
+        t = __builtin_fmaf(t, __builtin_fmaf(-lost, t, __builtin_fmaf(-d, t, 1.0f)), t);
+        float p = -0.020624879747629166f;
+        p = __builtin_fmaf(p, t, 0.11244352906942368f);
+        p = __builtin_fmaf(p, t, -0.22823289036750793f);
+        p = __builtin_fmaf(p, t, 0.19181127846240997f);
+        p = __builtin_fmaf(p, t, -0.07944672554731369f);
+        p = __builtin_fmaf(p, t, 0.09616988152265549f);
+        p = __builtin_fmaf(p, t, 0.07838491350412369f);
+        p = __builtin_fmaf(p, t, 0.11023649573326111f);
+        p = __builtin_fmaf(p, t, 0.11957168579101562f);
+        p = __builtin_fmaf(p, t, 0.11968670040369034f);
+        return p * t;
+    }
+    constexpr float k = 0x1p-32f;
+    float p = 0.03542373867332211f * k;
+    p = __builtin_fmaf(p, t, -0.1561584693838267f * k);
+    p = __builtin_fmaf(p, t, 0.20455683389817478f * k);
+    p = __builtin_fmaf(p, t, -0.05203407264399261f * k);
+    p = __builtin_fmaf(p, t, 0.12769180626590437f * k);
+    p = __builtin_fmaf(p, t, 0.10017593626445624f * k);
+    p = __builtin_fmaf(p, t, 0.1207121381245411f * k);
+    p = __builtin_fmaf(p, t, 0.1196320071032971f * k);
     return p * t;
 }
 
-// exp(-x^2 / 2) through the hardware's power of two.
-__device__ __forceinline__ float bell(float x) { return __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f); }
-
-// 2^32 sigmoid(x) for results of 16 bits, through the hardware's power of two and reciprocal.  Those know no numbers below 2^-126, which a
-// bf16 result can be made of: 2^32 brings everything that its type can hold into their range.  The exponent is rounded to fp32, which
-// costs |x| units of 2^-24 in the tail, 7e-6 at most, and up to 7e-7 near zero; a result rounds by 2^-9 or 2^-12.
+// Results of 16 bits: 2^32 exp(-x^2 / 2) and 2^32 sigmoid(x), through the hardware's power of two and reciprocal.  Those know no numbers
+// below 2^-126, which a bf16 result can be made of: 2^32 brings everything that its type can hold into their range.  The exponents are
+// rounded to fp32, which costs x^2 or |x| units of 2^-24 in the tails, 1.2e-5 at most, and up to 7e-7 near zero; a result rounds by 2^-9
+// or 2^-12.
+__device__ __forceinline__ float bellTimes2To32(float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x * x, -0.72134752044448170f, 32.0f)); }
 __device__ __forceinline__ float sigmoidTimes2To32(float x) {
     return __builtin_amdgcn_rcpf(0x1p-32f + __builtin_amdgcn_exp2f(__builtin_fmaf(x, -1.4426950408889634f, -32.0f)));
 }
@@ -111,14 +131,22 @@ __device__ __forceinline__ Power powerOfTwo(float hi, float lo) {
     const float whole = __builtin_rintf(hi);
     return {__builtin_amdgcn_exp2f(hi - whole + lo), (int)whole};
 }
-// exp(-a) for a in [0, 200]: log2(e) in two parts, and what the products lose.
+// exp(-a) for a in [0, 200], exp(-a^2 / 2) for a in [0, 100]: log2(e) in two parts, and what the products lose.
 __device__ __forceinline__ Power exponential(float a) {
 #pragma clang fp contract(off)
     const float hi = a * -1.44269502f;
     return powerOfTwo(hi, __builtin_fmaf(a, -1.92596303e-8f, __builtin_fmaf(a, -1.44269502f, -hi)));
 }
+__device__ __forceinline__ Power exactBell(float a) {
+#pragma clang fp contract(off)
+    const float square = a * a, hi = square * -0.721347511f;
+    float lo = __builtin_fmaf(square, -0.721347511f, -hi);
+    lo = __builtin_fmaf(square, -9.62981517e-9f, lo);
+    return powerOfTwo(hi, __builtin_fmaf(__builtin_fmaf(a, a, -square), -0.721347511f, lo));
+}
 
-// What the activations are made of at one x: f(x) of a finite x, f(x) of any x, and f'(x).
+// What the activations are made of at one x, in fp32 to some six units of 2^-24 (nine at most) down to the least number, in fewer
+// instructions for 16-bit results: f(x) of a finite x, f(x) of any x, and f'(x).
 template <typename T, int KIND>
 struct Activated;
 
@@ -157,17 +185,39 @@ struct Activated<float, THORHIP_SWISH> {
     __device__ __forceinline__ float slope() const { return __builtin_ldexpf(__builtin_fmaf(within * s, rest, s), exponent); }
 };
 
-// f = max(x, 0) - |x| Phi(-|x|), two instructions less than by cases (bf16 16384 x 8192 forward 126 -> 121 us: the one kernel
+// 16 bits: f = max(x, 0) - |x| Phi(-|x|), two instructions less than by cases (bf16 16384 x 8192 forward 126 -> 121 us: the one kernel
 // here that the vector units bound); f' = exp(-x^2 / 2) (H(|x|) - |x| / sqrt(2 pi)) below zero, and that from one above.
 template <typename T>
 struct Activated<T, THORHIP_GELU> {
-    float x, h, e;
-    __device__ __forceinline__ explicit Activated(float x) : x(x), h(tailFactor(__builtin_fabsf(x))), e(bell(x)) {}
+    float x, h, e;  // h / 2^32, 2^32 e
+    __device__ __forceinline__ explicit Activated(float x) : x(x), h(tailFactor<T>(__builtin_fabsf(x))), e(bellTimes2To32(x)) {}
     __device__ __forceinline__ float finite() const { return __builtin_fmaf(-__builtin_fabsf(x), h * e, __builtin_fmaxf(x, 0.0f)); }
     __device__ __forceinline__ float any() const { return x * phi(); }
     __device__ __forceinline__ float phi() const { return x < 0.0f ? h * e : 1.0f - h * e; }
     __device__ __forceinline__ float slope() const {
-        const float below = e * __builtin_fmaf(__builtin_fabsf(x), -0.39894228040143268f, h);
+        const float below = e * __builtin_fmaf(__builtin_fabsf(x), -0.39894228040143268f * 0x1p-32f, h);
+        return x < 0.0f ? below : 1.0f - below;
+    }
+};
+template <>
+struct Activated<float, THORHIP_GELU> {
+    float x, h;
+    Power e;
+    __device__ __forceinline__ explicit Activated(float x) : x(x) {
+        const float a = __builtin_amdgcn_fmed3f(__builtin_fabsf(x), 0.0f, 100.0f);
+        h = tailFactor<float>(a);
+        e = exactBell(a);
+    }
+    __device__ __forceinline__ float finite() const {
+        return __builtin_fmaxf(x, 0.0f) + e.times(-__builtin_fabsf(x) * (h * e.factor));
+    }
+    __device__ __forceinline__ float any() const { return x * phi(); }
+    __device__ __forceinline__ float phi() const {
+        const float below = e.times(h * e.factor);
+        return x < 0.0f ? below : 1.0f - below;
+    }
+    __device__ __forceinline__ float slope() const {
+        const float below = e.times(e.factor * __builtin_fmaf(__builtin_fabsf(x), -0.39894228040143268f, h));
         return x < 0.0f ? below : 1.0f - below;
     }
 };
@@ -251,18 +301,18 @@ __device__ __forceinline__ float finite(float x) {
 // gelu's slope, and Phi where there is a multiplier, at every value that a code of the two floating point formats can stand for.  Their
 // scales are powers of two, so such a value has a sign, an exponent and at most three bits more; the slope and Phi are 1/2 to the last
 // bit below 2^-26, and 0 or 1 to the last bit from 15 on.  That leaves 480 values, which a block of threads works out into shared memory
-// while its loads are on their way.  Without the table the kernel is bound by its vector instructions, some 28 slots per element with
-// the exponential and the reciprocal at a quarter of the rate: bf16 16384 x 8192 124.4 us, with it 103.0; with a multiplier 8192 x 8192
-// 90.3 and 84.8.  fp32 moves twice the bytes per element, has fewer of them per lane, and goes without; so do int8 codes, whose scales
-// are any number.
-template <bool PAIRS>
+// while its loads are on their way.  Without the table the kernel is bound by its vector instructions, some 28 slots per element in 16
+// bits and 45 in fp32 with the exponential and the reciprocal at a quarter of the rate: bf16 16384 x 8192 124.4 us, with it 103.0; with a
+// multiplier 8192 x 8192 90.3 and 84.8; fp32 8192 x 8192 103.5 and 96.4.  fp32 with a multiplier takes 159 either way and goes without,
+// as fp32's Phi has lost bits where x Phi has not; so do int8 codes, whose scales are any number.
+template <typename T, bool PAIRS>
 struct GeluTable {
     static constexpr u32 kFirst = (127 - 26) << 3, kLast = (127 + 3) << 3 | 7, kEntries = 2 * (kLast - kFirst + 1);
     static constexpr u32 kWidth = PAIRS ? 2 : 1, kFloats = kEntries * kWidth;
     __device__ static __forceinline__ void fill(float* table) {
         for (u32 i = threadIdx.x; i < kEntries; i += kThreads) {
             const float a = bitsF32((kFirst + i / 2) << 20);
-            const Activated<float, THORHIP_GELU> f(i % 2 != 0 ? -a : a);
+            const Activated<T, THORHIP_GELU> f(i % 2 != 0 ? -a : a);
             table[i * kWidth] = f.slope();
             if constexpr (PAIRS) table[i * kWidth + 1] = f.phi();
         }
@@ -285,9 +335,9 @@ __device__ __forceinline__ void backward(float dy, float& x, float& z) {
         z = dy * f.finite();
     }
 }
-template <bool MULTIPLIED>
+template <typename T, bool MULTIPLIED>
 __device__ __forceinline__ void backwardOfTable(const float* table, float dy, float& x, float& z) {
-    const float* entry = GeluTable<MULTIPLIED>::at(table, x);
+    const float* entry = GeluTable<T, MULTIPLIED>::at(table, x);
     if constexpr (MULTIPLIED) {
         const float f = x * entry[1];
         x = dy * z * entry[0];
@@ -347,11 +397,11 @@ __global__ __launch_bounds__(kThreads) void checkpointedBackward(CheckpointedArg
         p[u] = placeOf<VEC>(a, numberOfBlock() * TURNS + u);
         if (p[u].there) saved[u].load(a, p[u]);
     }
-    constexpr bool kTabled = KIND == THORHIP_GELU && sizeof(T) == 2;
-    __shared__ __attribute__((aligned(8))) float table[kTabled ? GeluTable<MULTIPLIED>::kFloats : 1];
+    constexpr bool kTabled = KIND == THORHIP_GELU && (sizeof(T) == 2 || !MULTIPLIED);
+    __shared__ __attribute__((aligned(8))) float table[kTabled ? GeluTable<T, MULTIPLIED>::kFloats : 1];
     const bool tabled = kTabled && a.format != THORHIP_INT8;
     if (tabled) {
-        GeluTable<MULTIPLIED>::fill(table);
+        GeluTable<T, MULTIPLIED>::fill(table);
         __syncthreads();
     }
 #pragma unroll
@@ -368,10 +418,12 @@ __global__ __launch_bounds__(kThreads) void checkpointedBackward(CheckpointedArg
             bool byTable = tabled && (f32Bits(s.xScale) & 0x7fffff) == 0;  // a power of two, as it is if the checkpoint was saved here
             if constexpr (KIND != THORHIP_IDENTITY) byTable = keepFinite(x) && byTable;
             if constexpr (MULTIPLIED) keepFinite(z);
+            if (byTable) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                if (byTable) backwardOfTable<MULTIPLIED>(table, dy[i], x[i], z[i]);
-                else backward<T, KIND, MULTIPLIED>(dy[i], x[i], z[i]);
+                for (int i = 0; i < VEC; ++i) backwardOfTable<T, MULTIPLIED>(table, dy[i], x[i], z[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) backward<T, KIND, MULTIPLIED>(dy[i], x[i], z[i]);
             }
             storeChunk(xOut + p[u].column, x);
             if constexpr (MULTIPLIED) storeChunk(zOut + p[u].column, z);
