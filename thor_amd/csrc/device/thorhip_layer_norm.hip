@@ -379,11 +379,12 @@ __global__ __launch_bounds__(kBackwardThreads<LANES>) void layerNormBackward(Bac
             }
             tail = widen(now.tailError);
             tailRow = now.tailRow(a);
-            tailWeightSum += at.tail ? tail * tailRow : 0.0f;  // elsewhere it may be a row's NaN
+            // where a lane has no element, h is 0 - mean times rstd, which may be no number
+            tailWeightSum += at.tail ? tail * tailRow : 0.0f;
             tailErrorSum += tail;
             tail *= tailWeight;
             sums[0] = tail;
-            sums[1] = tail * tailRow;
+            sums[1] = at.tail ? tail * tailRow : 0.0f;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 now.chunk(a, k, g[k], h[k]);
@@ -653,16 +654,19 @@ __global__ __launch_bounds__(1024) void layerNormBackwardFew(BackwardArgs a, u32
         tail = widen(now.tailError) * tailWeight;
         tailRow = now.tailRow(a);
         sums[0] = tail;
-        sums[1] = tail * tailRow;
+        sums[1] = at.tail ? tail * tailRow : 0.0f;  // where a lane has no element, h is 0 - mean times rstd, which may be no number
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             now.chunk(a, k, g[k], h[k]);
+            float ofChunk[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 g[k][i] *= weight[k][i];
-                sums[0] += g[k][i];
-                sums[1] += g[k][i] * h[k][i];
+                ofChunk[0] += g[k][i];
+                ofChunk[1] += g[k][i] * h[k][i];
             }
+            sums[0] += ofChunk[0];
+            sums[1] += at.has(k) ? ofChunk[1] : 0.0f;
         }
     }
     sumTeam<LANES>(sums, shared);
