@@ -46,3 +46,30 @@ def test_gradients_of_constant_rows_far_from_zero(stream, rows, cols, dtype):
     for got, value, o, what in zip(gradients_of(plans[0], stream), want, off, ("dx", "dweight", "dbias")):
         within(got, value, o, what)
     within(download(plans[1].get_input_gradient_tensor(), stream), want[0], off[0], "dx alone")
+
+
+@pytest.mark.parametrize("cols", [100, 1000, 9001, 16387])
+def test_the_mean_of_a_row_with_an_infinity(stream, cols):
+    """It is that infinity, or no number where there are both; the row's results are no numbers."""
+    x = np.random.default_rng(cols).standard_normal((4, cols)).astype(np.float32)
+    x[1, cols // 2], x[2, cols - 1], x[3, 0], x[3, 5] = np.inf, -np.inf, np.inf, -np.inf
+    tx, _ = upload(x, DataType.fp32, stream)
+    plan = ph.LayerNorm(EPSILON).stamp(tx, stream)
+    plan.run()
+    mean = download(plan.get_mean_tensor(), stream)[:, 0]
+    assert np.isfinite(mean[0]) and mean[1] == np.inf and mean[2] == -np.inf and np.isnan(mean[3])
+    assert np.isnan(download(plan.get_output_tensor(), stream)[1:]).all()
+
+
+@pytest.mark.parametrize("cols", [60, 1000, 9002, 16386, 40004])
+def test_squares_that_overflow(stream, cols):
+    """Differences of 2^100 have squares over fp32's range: rstd is zero and the output the bias, in rows of every length."""
+    x = np.where(np.arange(cols) % 2 == 0, 1.0, -1.0)[None].repeat(3, 0).astype(np.float32)
+    x[1] *= np.float32(2.0**100)
+    tx, _ = upload(x, DataType.fp32, stream)
+    tb, b = upload(np.random.default_rng(cols).standard_normal(cols), DataType.fp32, stream)
+    plan = ph.LayerNorm(EPSILON).stamp(tx, stream, bias=tb)
+    plan.run()
+    mean, rstd = download(plan.get_mean_tensor(), stream)[:, 0], download(plan.get_reciprocal_deviation_tensor(), stream)[:, 0]
+    assert not mean.any() and rstd[1] == 0 and np.isfinite(rstd).all()
+    assert np.array_equal(download(plan.get_output_tensor(), stream)[1], b)

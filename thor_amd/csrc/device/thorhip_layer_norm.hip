@@ -198,7 +198,7 @@ struct LongSum {
     float sum = 0.0f, lost = 0.0f;
     __device__ __forceinline__ void add(float x) {
         const float y = x - lost, t = sum + y;
-        lost = (t - sum) - y;
+        lost = __builtin_fabsf(t) < __builtin_inff() ? (t - sum) - y : 0.0f;  // an infinity stays one
         sum = t;
     }
 };
