@@ -4,9 +4,10 @@
 //   backward  input_gradient = error * f'(x), or error * z * f'(x), and multiplier_gradient = error * f(x), where x and z are what the
 //             checkpoints stand for (an infinity counts as the largest finite number there)
 // with f one of relu, gelu(x) = x * Phi(x) and swish(x) = x * sigmoid(x), as Expression's methods of these names; relu's slope at zero
-// is zero, and a NaN stays a NaN in value and slope.  All arithmetic is fp32, rounded once to the output's type: fp32 values are within ten
-// units of 2^-24 of f over the whole range, subnormal results included, and 16-bit ones within 2e-5 before their rounding.  The tensors of a call
-// share one shape and one of the types FP32, FP16, BF16; strides, segment_offsets, overlaps and errors as in ActivationCheckpoint.h.
+// is zero, and a NaN stays a NaN in value and slope.  All arithmetic is fp32, rounded once to the output's type: fp32 values are within
+// ten units of 2^-24 of f over the whole range, subnormal results included, and 16-bit ones within 2e-5 before their rounding.  The tensors
+// of a call share one shape and one of the types FP32, FP16, BF16; strides, segment_offsets, overlaps and errors as in
+// ActivationCheckpoint.h.
 #pragma once
 
 #include "Utilities/TensorOperations/DataTypeConversions/ActivationCheckpoint.h"

@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 
 from helpers import copy_gpu_to_numpy
-from row_operations import UNIT, download, layer_norm_gradient_tolerances, layer_norm_gradients, upload, within
+from row_operations import (CHAIN, UNIT, decode, download, half_step_of_code, layer_norm, layer_norm_gradient_tolerances, layer_norm_gradients, rounding,
+                            upload, within)
 from thor_amd import physical as ph
 from thor_amd.dtypes import DataType
 
@@ -46,6 +47,58 @@ def test_gradients_of_constant_rows_far_from_zero(stream, rows, cols, dtype):
     for got, value, o, what in zip(gradients_of(plans[0], stream), want, off, ("dx", "dweight", "dbias")):
         within(got, value, o, what)
     within(download(plans[1].get_input_gradient_tensor(), stream), want[0], off[0], "dx alone")
+
+
+# every form of the forward pass: teams of 16 to 1024 lanes, rows with and without a tail, of whole chunks, whole blocks and full ones,
+# of any length; rows in turn
+MEANS = [(3, 7, DataType.fp32), (40, 128, DataType.bf16), (5, 200, DataType.fp32), (9, 512, DataType.fp16), (4, 1000, DataType.fp32), (3, 2048, DataType.bf16),
+         (3, 2569, DataType.fp32), (5, 4096, DataType.fp32), (3, 6664, DataType.fp16), (2, 8192, DataType.fp32), (3, 11008, DataType.bf16), (2, 16384, DataType.fp32),
+         (3, 16387, DataType.fp32), (2, 40000, DataType.fp32), (9000, 60, DataType.fp32), (2600, 1537, DataType.fp32)]
+
+
+@pytest.mark.parametrize("rows,cols,dtype", MEANS, ids=[f"{r}x{c}-{d.name}" for r, c, d in MEANS])
+def test_means_that_are_large_against_the_deviation(stream, rows, cols, dtype):
+    """h and rstd have the precision of differences from the mean: CHAIN roundings of these, however large the mean is.  The differences are
+    from the mean as its sum's CHAIN roundings leave it, which is where the tolerance's second part is from.  16-bit rows up to some
+    length keep the mean as it is: their h moves by its roundings, and the variance by their square."""
+    rng = np.random.default_rng([rows, cols, 1])
+    x = rng.standard_normal((rows, cols)) + np.where(np.arange(rows) % 3 == 0, 1.0, np.where(np.arange(rows) % 3 == 1, -300.0, 6e4 / 8))[:, None]
+    if dtype == DataType.fp32:
+        x[-1] += 65536.0
+    tx, x = upload(x, dtype, stream)
+    tw, w = upload(1 + 0.2 * rng.standard_normal(cols), DataType.fp32, stream)
+    tb, b = upload(0.1 * rng.standard_normal(cols), DataType.fp32, stream)
+    plan = ph.LayerNorm(EPSILON, DataType.fp8_e4m3).stamp(tx, stream, weight=tw, bias=tb)
+    plan.run()
+    y, mean, rstd, h = layer_norm(x, w, b, EPSILON)
+    from_near = CHAIN * UNIT * np.abs(x).mean(1, keepdims=True)  # how far the value that differences are taken from may be off the mean
+    refined = dtype == DataType.fp32 or cols > (6144 if dtype == DataType.fp16 else 16384)
+    mean_off = CHAIN * UNIT * (np.abs(x - mean).mean(1, keepdims=True) + from_near) if refined else from_near
+    rstd_off = rstd * (CHAIN * UNIT * (1 + (from_near * rstd)**2) + (0.0 if refined else (from_near * rstd)**2))
+    h_off = rstd * mean_off + np.abs(h) * (rstd_off / rstd + 4 * UNIT) + 2 * UNIT * rstd * from_near
+    y_off = np.abs(w) * h_off + 4 * UNIT * (np.abs(h * w) + np.abs(b))
+    within(download(plan.get_mean_tensor(), stream), mean, mean_off + rounding(mean, DataType.fp32), "mean")
+    within(download(plan.get_reciprocal_deviation_tensor(), stream), rstd, rstd_off, "rstd")
+    within(download(plan.get_output_tensor(), stream), y, y_off + rounding(np.abs(y) + y_off, dtype), "y")
+    scales = copy_gpu_to_numpy(plan.get_checkpoint().scales, stream)
+    kept = decode(copy_gpu_to_numpy(plan.get_checkpoint().codes, stream), scales, DataType.fp8_e4m3).astype(np.float64)
+    within(kept, h, h_off + half_step_of_code(np.abs(h) + h_off, scales, DataType.fp8_e4m3), "restored")
+
+
+@pytest.mark.parametrize("dtype,cols", [(DataType.fp16, 37), (DataType.fp16, 4096), (DataType.bf16, 6144), (DataType.fp16, 6143), (DataType.fp16, 8191), (DataType.bf16, 16384),
+                                        (DataType.fp16, 12003), (DataType.fp32, 130), (DataType.fp32, 4099), (DataType.fp32, 16384), (DataType.fp16, 20001),
+                                        (DataType.fp32, 50003)])
+def test_constant_rows_are_zero_before_the_bias(stream, dtype, cols):
+    """Exactly where the sums are exact, in bf16, and in fp16 up to 6144 columns.  Elsewhere a mean that is off by a last bit is refined: what is left
+    of x - mean is CHAIN roundings of a difference that is CHAIN roundings of x, and rstd is at most 1 / sqrt(epsilon)."""
+    values = np.array([2047.0, -1.0009765625, 37.28125, 0.333251953125, 60000.0 if dtype == DataType.fp16 else 123456.0])
+    tx, x = upload(np.repeat(values[:, None], cols, 1), dtype, stream)
+    plan = ph.LayerNorm(EPSILON).stamp(tx, stream)
+    plan.run()
+    y = download(plan.get_output_tensor(), stream)
+    if dtype == DataType.bf16 or (dtype == DataType.fp16 and cols <= 6144):
+        assert not y.any() and np.array_equal(download(plan.get_mean_tensor(), stream), x[:, :1])
+    within(y, np.zeros_like(x), np.broadcast_to((CHAIN * UNIT)**2 * np.abs(x) / np.sqrt(EPSILON), x.shape), "y")
 
 
 @pytest.mark.parametrize("cols", [100, 1000, 9001, 16387])

@@ -1,8 +1,8 @@
 // Layer norm over the last axis, forward and backward.
 //
 // Forward, one row: mean = sum x / C, rstd = 1 / sqrt(sum (x - mean)^2 / C + epsilon), y = (x - mean) * rstd * weight + bias.  A row is
-// read once and stays in registers between the two sums and the output; the squares are those of differences, so that a mean that is
-// large against the deviation costs no precision.  Everything is fp32, rounded once where it is stored.
+// read once and stays in registers between the two sums and the output; the squares are those of differences from the mean, and where the
+// mean's rounding could be seen in h the sum of these differences makes up for it.  Everything is fp32, rounded once where it is stored.
 //
 // Backward, one row, with h = (x - mean) * rstd and g = dy * weight:
 //   dx = rstd * (g - sum(g) / C - h * sum(g * h) / C),  weight gradient = sum over rows of dy * h,  bias gradient = sum over rows of dy.
@@ -14,6 +14,7 @@
 #include "thorhip_rows.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -73,9 +74,31 @@ __device__ __forceinline__ float average(float sum, u32 columns, float inverse) 
     const float q = sum * inverse, left = __builtin_fmaf(-q, (float)columns, sum);
     return __builtin_fmaf(__builtin_fminf(left, 3.40282347e38f), inverse, q);  // an infinite sum leaves no number
 }
-// 1 / sqrt(squares / columns + epsilon), one unit off at most where its argument is a normal number, which epsilon sees to.
-__device__ __forceinline__ float reciprocalDeviation(float squares, const ForwardArgs& a) {
-    return __builtin_amdgcn_rsqf(__builtin_fmaf(squares, a.inverse, a.epsilon));
+// Whether a row's mean is refined by the sum of the differences from it.  A mean rounds to its own last bits, which are many of the
+// deviation's where it is large against that: fp32 rows around 4096 with a deviation of one have an h that is off by 4e-4 without, 5e-7
+// with it.  16-bit rows do without as long as sums of equal elements are exact, 8 bits each of bf16 and 11 of up to 6144 of fp16: a row
+// of one value is zero then, and where the elements differ, their own last bits are 2^13 times the mean's at least.  There it would cost
+// time (16380 x 4097 61.0 us, without 55.8; 262144 x 96 18.2 and 17.0; 8192 x 8192 46.6 and 44.7), while fp32 takes the same either way
+// (32768 x 1024 43.9 us, 16380 x 4097 106, 8192 x 8192 99).
+template <typename T, int LANES>
+constexpr bool kRefined = sizeof(T) == 4 || (std::is_same<T, f16>::value && LANES >= 512);
+
+// A row's mean and 1 / sqrt(variance + epsilon) (the hardware's reciprocal root, one unit off at most where its argument is a normal
+// number, which epsilon sees to), from a value near the mean, the sum of the squares of the differences from it, and the sum of these.
+struct Moments {
+    float mean, rstd, shift;
+    __device__ __forceinline__ float normalised(float difference) const { return __builtin_fmaf(difference, rstd, shift); }
+};
+__device__ __forceinline__ Moments momentsOf(float near, const float (&sums)[1], const ForwardArgs& a) {
+    return {near, __builtin_amdgcn_rsqf(__builtin_fmaf(sums[0], a.inverse, a.epsilon)), 0.0f};
+}
+__device__ __forceinline__ Moments momentsOf(float near, const float (&sums)[2], const ForwardArgs& a) {
+    constexpr float kMost = 3.40282347e38f;
+    // of a row with an infinity the differences are no numbers, but its mean is one; squares that overflow, or are no numbers, stay
+    const float left = __builtin_amdgcn_fmed3f(sums[1] * a.inverse, -kMost, kMost);
+    const float squares = sums[0] < __builtin_inff() ? __builtin_fmaxf(__builtin_fmaf(-left, sums[1], sums[0]), 0.0f) : sums[0];
+    const float rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(squares, a.inverse, a.epsilon));
+    return {near + left, rstd, -left * rstd};
 }
 
 // The team of a block that a lane is in; the compiler is told that it is the same for a wavefront.
@@ -109,7 +132,8 @@ __device__ __forceinline__ void loadsArrived() { __builtin_amdgcn_s_waitcnt(0x0f
 template <typename T, int LANES, int K, bool CHECKPOINT, Fit FIT>
 __global__ __launch_bounds__(kForwardThreads<LANES>) void layerNormForward(ForwardArgs a) {
     constexpr int VEC = kVec<T>, TEAMS = kForwardThreads<LANES> / LANES;
-    __shared__ float shared[2][LANES / 64 + 1][1];
+    constexpr bool REFINED = kRefined<T, LANES>;
+    __shared__ float shared[LANES / 64 + 1][1], sharedOfDifferences[LANES / 64 + 1][REFINED ? 2 : 1];
     const RowLayout<T, LANES, FIT> at(a.columns, threadIdx.x % LANES);
     // a lane without a chunk works on another's where the whole block of codes does; elsewhere the block's scale would not be the same
     const auto works = [&](int k) { return FIT == Fit::Blocks || at.has(k); };
@@ -149,34 +173,38 @@ __global__ __launch_bounds__(kForwardThreads<LANES>) void layerNormForward(Forwa
             for (int i = 0; i < VEC; ++i) ofChunk += x[k][i];
             sum[0] += at.has(k) ? ofChunk : 0.0f;
         }
-        sumTeam<LANES>(sum, shared[0]);
-        const float mean = average(sum[0], a.columns, a.inverse);
-        tail -= mean;
-        float squares[1] = {at.tail ? tail * tail : 0.0f};
+        sumTeam<LANES>(sum, shared);
+        const float near = average(sum[0], a.columns, a.inverse);
+        tail -= near;
+        float sums[REFINED ? 2 : 1];
+        sums[0] = at.tail ? tail * tail : 0.0f;
+        if constexpr (REFINED) sums[1] = at.tail ? tail : 0.0f;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            float ofChunk = 0.0f;
+            float ofChunk[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                x[k][i] -= mean;
-                ofChunk += x[k][i] * x[k][i];
+                x[k][i] -= near;
+                ofChunk[0] += x[k][i] * x[k][i];
+                if constexpr (REFINED) ofChunk[1] += x[k][i];
             }
-            squares[0] += at.has(k) ? ofChunk : 0.0f;
+            sums[0] += at.has(k) ? ofChunk[0] : 0.0f;
+            if constexpr (REFINED) sums[1] += at.has(k) ? ofChunk[1] : 0.0f;
         }
-        sumTeam<LANES>(squares, shared[1]);
-        const float rstd = reciprocalDeviation(squares[0], a);
+        sumTeam<LANES>(sums, sharedOfDifferences);
+        const Moments m = momentsOf(near, sums, a);
         if (at.lane == 0) {
-            a.mean[row] = mean;
-            a.rstd[row] = rstd;
+            a.mean[row] = m.mean;
+            a.rstd[row] = m.rstd;
         }
         T* out = rowPointer<T>(a.output, row, a.innerRows);
         u8* codes = a.codes + (i64)row * a.columns;
         float* scales = a.scales + (i64)row * a.blocksPerRow;
-        tail *= rstd;
+        tail = REFINED ? m.normalised(tail) : tail * m.rstd;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) x[k][i] *= rstd;
+            for (int i = 0; i < VEC; ++i) x[k][i] = REFINED ? m.normalised(x[k][i]) : x[k][i] * m.rstd;
             if constexpr (CHECKPOINT) {
                 const bool hasTail = at.tail && k == at.tailChunk;
                 const BlockScale scale = scaleOfLanes<VEC>(x[k], works(k), tail, hasTail, a.format);
@@ -208,7 +236,7 @@ struct LongSum {
 template <typename T, bool CHECKPOINT>
 __global__ __launch_bounds__(1024) void layerNormForwardLong(ForwardArgs a) {
     constexpr int VEC = kVec<T>, LANES = 1024;
-    __shared__ float shared[2][LANES / 64][1];
+    __shared__ float shared[LANES / 64][1], sharedOfDifferences[LANES / 64][2];
     const RowLayout<T, LANES, Fit::Any> at(a.columns, threadIdx.x);
     const u32 rows = rowsInUse(a.extent);
     for (u32 row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -223,28 +251,32 @@ __global__ __launch_bounds__(1024) void layerNormForwardLong(ForwardArgs a) {
             ofLane.add(ofChunk);
         }
         float sum[1] = {ofLane.sum + tail};
-        sumTeam<LANES>(sum, shared[0]);
-        const float mean = average(sum[0], a.columns, a.inverse);
-        tail -= mean;
-        LongSum squaresOfLane;
+        sumTeam<LANES>(sum, shared);
+        const float near = average(sum[0], a.columns, a.inverse);
+        tail -= near;
+        LongSum squaresOfLane, differencesOfLane;
         for (int k = 0; at.has(k); ++k) {
             loadChunk(in + at.column(k), x);
-            float ofChunk = 0.0f;
+            float ofChunk[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) ofChunk += (x[i] - mean) * (x[i] - mean);
-            squaresOfLane.add(ofChunk);
+            for (int i = 0; i < VEC; ++i) {
+                ofChunk[0] += (x[i] - near) * (x[i] - near);
+                ofChunk[1] += x[i] - near;
+            }
+            squaresOfLane.add(ofChunk[0]);
+            differencesOfLane.add(ofChunk[1]);
         }
-        float squares[1] = {squaresOfLane.sum + (at.tail ? tail * tail : 0.0f)};
-        sumTeam<LANES>(squares, shared[1]);
-        const float rstd = reciprocalDeviation(squares[0], a);
+        float sums[2] = {squaresOfLane.sum + (at.tail ? tail * tail : 0.0f), differencesOfLane.sum + (at.tail ? tail : 0.0f)};
+        sumTeam<LANES>(sums, sharedOfDifferences);
+        const Moments m = momentsOf(near, sums, a);
         if (threadIdx.x == 0) {
-            a.mean[row] = mean;
-            a.rstd[row] = rstd;
+            a.mean[row] = m.mean;
+            a.rstd[row] = m.rstd;
         }
         T* out = rowPointer<T>(a.output, row, a.innerRows);
         u8* codes = a.codes + (i64)row * a.columns;
         float* scales = a.scales + (i64)row * a.blocksPerRow;
-        tail *= rstd;
+        tail = m.normalised(tail);
         const int steps = (a.columns + LANES * VEC - 1) / (LANES * VEC);  // the same for all lanes of a block of codes
         for (int k = 0; k < steps; ++k) {
             const bool has = at.has(k);
@@ -253,7 +285,7 @@ __global__ __launch_bounds__(1024) void layerNormForwardLong(ForwardArgs a) {
             if (has) {
                 loadChunk(in + at.column(k), x);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) x[i] = (x[i] - mean) * rstd;
+                for (int i = 0; i < VEC; ++i) x[i] = m.normalised(x[i] - near);
             }
             if constexpr (CHECKPOINT) {
                 const bool hasTail = at.tail && k == at.tailChunk;
