@@ -126,3 +126,20 @@ def test_squares_that_overflow(stream, cols):
     mean, rstd = download(plan.get_mean_tensor(), stream)[:, 0], download(plan.get_reciprocal_deviation_tensor(), stream)[:, 0]
     assert not mean.any() and rstd[1] == 0 and np.isfinite(rstd).all()
     assert np.array_equal(download(plan.get_output_tensor(), stream)[1], b)
+
+
+@pytest.mark.parametrize("rows,cols", [(1 << 23, 4), (1 << 19, 2052), (7 << 14, 16400)])
+def test_parameter_gradients_over_many_rows(stream, rows, cols):
+    """A sum over rows has CHAIN roundings at most, however many rows there are.  The rows are one value, of which an addition to a sum
+    between 512 and 1024 loses 0.49 of a last bit every time: a chain of 1024 rows would be off by 240 roundings."""
+    value = np.float32(1 + 0.49 * 2.0**-14)
+    one, _ = upload(np.ones((1, cols)), DataType.fp32, stream)
+    error, _ = upload(np.full((1, cols), value), DataType.fp32, stream)
+    mean, _ = upload(np.zeros((rows, 1)), DataType.fp32, stream)
+    rstd, _ = upload(np.ones((rows, 1)), DataType.fp32, stream)
+    everywhere = lambda t: t.alias_view([rows, cols], [0, 1])  # noqa: E731
+    plan = ph.LayerNormBackward().stamp(everywhere(error), everywhere(one), rstd, stream, mean=mean)
+    plan.run()
+    want = np.full(cols, rows * np.float64(value))
+    for got in (plan.get_weight_gradient_tensor(), plan.get_bias_gradient_tensor()):
+        within(download(got, stream), want, (CHAIN + 1) * UNIT * want, "sum over rows")

@@ -46,9 +46,14 @@ struct BackwardArgs {
     void* biasGradient;
     Extent extent;
     u32 columns, innerRows, blocksPerRow;
+    u32 sharesOfBlock;  // of the partials: one for each kRowsOfShare rows of a team
     int parametersAreFloat, format;
     float inverse;  // 1 / columns
 };
+
+// Rows that a lane adds up for a parameter gradient one after the other, at most.  A block that takes more of them begins another share,
+// and the sums over shares are compensated, so that a gradient over millions of rows has the error of one over some thousands.
+constexpr u32 kRowsOfShare = 128;
 
 template <typename T>
 __device__ __forceinline__ void loadParameters(const void* p, int isFloat, float missing, u32 column, bool has, float (&v)[kVec<T>]) {
@@ -384,7 +389,7 @@ __device__ __forceinline__ Elements<float> quarter(const float (&v)[K][VEC], int
 template <typename T, int LANES, int K, bool CODES, Fit FIT>
 __global__ __launch_bounds__(kBackwardThreads<LANES>) void layerNormBackward(BackwardArgs a) {
     constexpr int VEC = kVec<T>, THREADS = kBackwardThreads<LANES>, TEAMS = THREADS / LANES;
-    constexpr bool AHEAD = LANES < 1024;  // 128 registers per lane are too few for the next row and the weights
+    constexpr bool AHEAD = LANES < 1024;  // of 128 registers per lane this row takes 112 to 128
     __shared__ float shared[2][THREADS / 64][2];
     const RowLayout<T, LANES, FIT> at(a.columns, threadIdx.x % LANES);
     const u32 team = teamOfBlock<LANES>(), rows = rowsInUse(a.extent), step = gridDim.x * TEAMS;
@@ -398,122 +403,134 @@ __global__ __launch_bounds__(kBackwardThreads<LANES>) void layerNormBackward(Bac
     float tailWeightSum = 0.0f, tailErrorSum = 0.0f;
     loadsArrived();
     int turn = 0;
-    // The teams of a block take their turns together: those of several wavefronts synchronise.
-    for (u32 first = blockIdx.x * TEAMS; first < rows; first += step, row += step) {
-        const bool mine = row < rows;
-        float h[K][VEC], g[K][VEC], tail = 0.0f, tailRow = 0.0f;
-        float sums[2] = {0.0f, 0.0f};
-        if (mine) {
-            if constexpr (AHEAD) {
-                if (row + step < rows) next.load(a, at, row + step);
-            } else {
-                now.load(a, at, row);
-            }
-            tail = widen(now.tailError);
-            tailRow = now.tailRow(a);
-            // where a lane has no element, h is 0 - mean times rstd, which may be no number
-            tailWeightSum += at.tail ? tail * tailRow : 0.0f;
-            tailErrorSum += tail;
-            tail *= tailWeight;
-            sums[0] = tail;
-            sums[1] = at.tail ? tail * tailRow : 0.0f;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                now.chunk(a, k, g[k], h[k]);
-                if constexpr (!AHEAD) loadParameters<T>(a.weight, a.parametersAreFloat, 1.0f, at.source(k), at.works(k), weight[k]);
-                float ofChunk[2] = {0.0f, 0.0f};
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    weightSum[k][i] += g[k][i] * h[k][i];
-                    errorSum[k][i] += g[k][i];
-                    g[k][i] *= weight[k][i];
-                    ofChunk[0] += g[k][i];
-                    ofChunk[1] += g[k][i] * h[k][i];
+    u32 first = blockIdx.x * TEAMS;
+    for (u32 share = 0; share < a.sharesOfBlock; ++share) {
+        // The teams of a block take their turns together: those of several wavefronts synchronise.
+        for (u32 turns = a.sharesOfBlock == 1 ? ~0u : kRowsOfShare; first < rows && turns != 0; first += step, row += step, --turns) {
+            const bool mine = row < rows;
+            float h[K][VEC], g[K][VEC], tail = 0.0f, tailRow = 0.0f;
+            float sums[2] = {0.0f, 0.0f};
+            if (mine) {
+                if constexpr (AHEAD) {
+                    if (row + step < rows) next.load(a, at, row + step);
+                } else {
+                    now.load(a, at, row);
                 }
-                sums[0] += at.has(k) ? ofChunk[0] : 0.0f;
-                sums[1] += at.has(k) ? ofChunk[1] : 0.0f;
-            }
-        }
-        sumTeam<LANES>(sums, shared[turn]);
-        turn ^= 1;
-        if (mine) {
-            const float ofError = average(sums[0], a.columns, a.inverse), ofProduct = average(sums[1], a.columns, a.inverse);
-            T* out = rowPointer<T>(a.gradient, row, a.innerRows);
+                tail = widen(now.tailError);
+                tailRow = now.tailRow(a);
+                // where a lane has no element, h is 0 - mean times rstd, which may be no number
+                tailWeightSum += at.tail ? tail * tailRow : 0.0f;
+                tailErrorSum += tail;
+                tail *= tailWeight;
+                sums[0] = tail;
+                sums[1] = at.tail ? tail * tailRow : 0.0f;
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
+                for (int k = 0; k < K; ++k) {
+                    now.chunk(a, k, g[k], h[k]);
+                    if constexpr (!AHEAD) loadParameters<T>(a.weight, a.parametersAreFloat, 1.0f, at.source(k), at.works(k), weight[k]);
+                    float ofChunk[2] = {0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) g[k][i] = now.rstd * (g[k][i] - ofError - h[k][i] * ofProduct);
-                if (at.works(k)) storeChunk(out + at.source(k), g[k]);
-            }
-            if (at.tail) out[at.tailColumn] = narrow<T>(now.rstd * (tail - ofError - tailRow * ofProduct));
-            if constexpr (AHEAD) {
-                __builtin_amdgcn_sched_barrier(0);  // the stores first: what is copied here has to have arrived
-                now = next;
-            }
-        }
-    }
-    if (a.partials == nullptr) return;
-    float* mine = a.partials + (i64)blockIdx.x * 2 * a.columns;
-    if constexpr (TEAMS > 1) {
-        // The upper half of the teams gives its sums to the lower half until one team has them all; the block stores them together, 16
-        // adjacent bytes per lane.
-        constexpr u32 PARTS = K * VEC / 4, ROW = LANES * VEC / 4;
-        __shared__ Words4 given[TEAMS / 2][2][PARTS][LANES];
-        __shared__ float givenTail[TEAMS / 2][2][FIT == Fit::Any ? LANES : 1];
-        const u32 lane = threadIdx.x % LANES;
-        const auto give = [&](u32 to) {
-#pragma unroll
-            for (u32 q = 0; q < PARTS; ++q) {
-                given[to][0][q][lane] = __builtin_bit_cast(Words4, quarter(weightSum, q));
-                given[to][1][q][lane] = __builtin_bit_cast(Words4, quarter(errorSum, q));
-            }
-        };
-#pragma unroll
-        for (u32 half = TEAMS / 2; half >= 1; half /= 2) {
-            if (team >= half && team < 2 * half) {
-                give(team - half);
-                if constexpr (FIT == Fit::Any) {
-                    givenTail[team - half][0][lane] = tailWeightSum;
-                    givenTail[team - half][1][lane] = tailErrorSum;
+                    for (int i = 0; i < VEC; ++i) {
+                        weightSum[k][i] += g[k][i] * h[k][i];
+                        errorSum[k][i] += g[k][i];
+                        g[k][i] *= weight[k][i];
+                        ofChunk[0] += g[k][i];
+                        ofChunk[1] += g[k][i] * h[k][i];
+                    }
+                    sums[0] += at.has(k) ? ofChunk[0] : 0.0f;
+                    sums[1] += at.has(k) ? ofChunk[1] : 0.0f;
                 }
             }
-            __syncthreads();
-            if (team < half) {
+            sumTeam<LANES>(sums, shared[turn]);
+            turn ^= 1;
+            if (mine) {
+                const float ofError = average(sums[0], a.columns, a.inverse), ofProduct = average(sums[1], a.columns, a.inverse);
+                T* out = rowPointer<T>(a.gradient, row, a.innerRows);
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) g[k][i] = now.rstd * (g[k][i] - ofError - h[k][i] * ofProduct);
+                    if (at.works(k)) storeChunk(out + at.source(k), g[k]);
+                }
+                if (at.tail) out[at.tailColumn] = narrow<T>(now.rstd * (tail - ofError - tailRow * ofProduct));
+                if constexpr (AHEAD) {
+                    __builtin_amdgcn_sched_barrier(0);  // the stores first: what is copied here has to have arrived
+                    now = next;
+                }
+            }
+        }
+        if (a.partials == nullptr) return;
+        float* mine = a.partials + ((i64)share * gridDim.x + blockIdx.x) * 2 * a.columns;
+        if constexpr (TEAMS > 1) {
+            // The upper half of the teams gives its sums to the lower half until one team has them all; the block stores them together, 16
+            // adjacent bytes per lane.
+            constexpr u32 PARTS = K * VEC / 4, ROW = LANES * VEC / 4;
+            __shared__ Words4 given[TEAMS / 2][2][PARTS][LANES];
+            __shared__ float givenTail[TEAMS / 2][2][FIT == Fit::Any ? LANES : 1];
+            u32 thread = threadIdx.x;
+            asm volatile("" : "+v"(thread));  // what follows from it is worked out here and takes no registers from the rows
+            const u32 lane = thread % LANES;
+            const auto give = [&](u32 to) {
 #pragma unroll
                 for (u32 q = 0; q < PARTS; ++q) {
-                    const Elements<float> w = __builtin_bit_cast(Elements<float>, given[team][0][q][lane]);
-                    const Elements<float> e = __builtin_bit_cast(Elements<float>, given[team][1][q][lane]);
+                    given[to][0][q][lane] = __builtin_bit_cast(Words4, quarter(weightSum, q));
+                    given[to][1][q][lane] = __builtin_bit_cast(Words4, quarter(errorSum, q));
+                }
+            };
 #pragma unroll
-                    for (u32 i = 0; i < 4; ++i) {
-                        weightSum[q * 4 / VEC][q * 4 % VEC + i] += w.e[i];
-                        errorSum[q * 4 / VEC][q * 4 % VEC + i] += e.e[i];
+            for (u32 half = TEAMS / 2; half >= 1; half /= 2) {
+                if (team >= half && team < 2 * half) {
+                    give(team - half);
+                    if constexpr (FIT == Fit::Any) {
+                        givenTail[team - half][0][lane] = tailWeightSum;
+                        givenTail[team - half][1][lane] = tailErrorSum;
                     }
                 }
-                if constexpr (FIT == Fit::Any) {
-                    tailWeightSum += givenTail[team][0][lane];
-                    tailErrorSum += givenTail[team][1][lane];
+                __syncthreads();
+                if (team < half) {
+#pragma unroll
+                    for (u32 q = 0; q < PARTS; ++q) {
+                        const Elements<float> w = __builtin_bit_cast(Elements<float>, given[team][0][q][lane]);
+                        const Elements<float> e = __builtin_bit_cast(Elements<float>, given[team][1][q][lane]);
+#pragma unroll
+                        for (u32 i = 0; i < 4; ++i) {
+                            weightSum[q * 4 / VEC][q * 4 % VEC + i] += w.e[i];
+                            errorSum[q * 4 / VEC][q * 4 % VEC + i] += e.e[i];
+                        }
+                    }
+                    if constexpr (FIT == Fit::Any) {
+                        tailWeightSum += givenTail[team][0][lane];
+                        tailErrorSum += givenTail[team][1][lane];
+                    }
+                    if (half == 1) give(0);
                 }
-                if (half == 1) give(0);
+                __syncthreads();
             }
-            __syncthreads();
+            for (u32 t = thread; t < 2 * K * ROW; t += THREADS) {
+                const u32 which = t / (K * ROW), k = t / ROW % K, of = t % ROW / (VEC / 4), q = k * (VEC / 4) + t % (VEC / 4);
+                const u32 column = t % (K * ROW) * 4;
+                if (column < at.whole) *reinterpret_cast<Words4OfFloats*>(mine + which * a.columns + column) = given[0][which][q][of];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!at.has(k)) continue;
+                storeFloats<VEC>(mine + at.column(k), weightSum[k]);
+                storeFloats<VEC>(mine + a.columns + at.column(k), errorSum[k]);
+            }
         }
-        for (u32 t = threadIdx.x; t < 2 * K * ROW; t += THREADS) {
-            const u32 which = t / (K * ROW), k = t / ROW % K, of = t % ROW / (VEC / 4), q = k * (VEC / 4) + t % (VEC / 4);
-            const u32 column = t % (K * ROW) * 4;
-            if (column < at.whole) *reinterpret_cast<Words4OfFloats*>(mine + which * a.columns + column) = given[0][which][q][of];
+        if (at.tail && team == 0) {
+            mine[at.tailColumn] = tailWeightSum;
+            mine[a.columns + at.tailColumn] = tailErrorSum;
         }
-        if (team != 0) return;
-    } else {
+        if (share + 1 == a.sharesOfBlock) return;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            if (!at.has(k)) continue;
-            storeFloats<VEC>(mine + at.column(k), weightSum[k]);
-            storeFloats<VEC>(mine + a.columns + at.column(k), errorSum[k]);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) weightSum[k][i] = errorSum[k][i] = 0.0f;
         }
-    }
-    if (at.tail) {
-        mine[at.tailColumn] = tailWeightSum;
-        mine[a.columns + at.tailColumn] = tailErrorSum;
+        tailWeightSum = tailErrorSum = 0.0f;
+        if constexpr (TEAMS > 1) __syncthreads();  // what the teams gave each other has been read
     }
 }
 
@@ -729,25 +746,25 @@ __global__ __launch_bounds__(1024) void addShares(const float* partials, u32 sha
     const u32 column = blockIdx.x * 32 + threadIdx.x % 8 * 4, wave = threadIdx.x / 64;
     W* out = blockIdx.y == 0 ? weightGradient : biasGradient;
     if (out == nullptr) return;
-    float sum[4] = {};
+    LongSum sums[4];
     if (column + 4 <= columns) {
 #pragma unroll 4
         for (u32 s = threadIdx.x / 8; s < shares; s += 128) {
             const Elements<float> x = __builtin_bit_cast(Elements<float>, *reinterpret_cast<const Words4OfFloats*>(partials + ((i64)s * 2 + blockIdx.y) * columns + column));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] += x.e[i];
+            for (int i = 0; i < 4; ++i) sums[i].add(x.e[i]);
         }
     } else {
         for (u32 s = threadIdx.x / 8; s < shares; s += 128) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (column + i < columns) sum[i] += partials[((i64)s * 2 + blockIdx.y) * columns + column + i];
+                if (column + i < columns) sums[i].add(partials[((i64)s * 2 + blockIdx.y) * columns + column + i]);
         }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // the eight shares of a wavefront
-        sum[i] = sumRowsOfWave(sum[i] + bitsF32(rotated<0x128>(f32Bits(sum[i]))));
-        if (threadIdx.x % 64 < 8) added[wave][threadIdx.x % 8 * 4 + i] = sum[i];
+        const float sum = sumRowsOfWave(sums[i].sum + bitsF32(rotated<0x128>(f32Bits(sums[i].sum))));
+        if (threadIdx.x % 64 < 8) added[wave][threadIdx.x % 8 * 4 + i] = sum;
     }
     __syncthreads();
     const u32 mine = blockIdx.x * 32 + threadIdx.x;
@@ -1016,6 +1033,7 @@ int thorhip_layer_norm_backward(const thorhip_layer_norm_gradient* call, void* s
     a.parametersAreFloat = c.parameter_dtype == THORHIP_FP32;
     a.format = c.checkpoint_dtype;
     a.inverse = 1.0f / (float)c.columns;
+    a.sharesOfBlock = 1;
     const bool parameters = c.weight_gradient != nullptr || c.bias_gradient != nullptr;
     const int vec = 16 / thorhip_dtype_size(c.dtype);
     a.weightGradient = c.weight_gradient;
@@ -1049,11 +1067,14 @@ int thorhip_layer_norm_backward(const thorhip_layer_norm_gradient* call, void* s
         // One block of eight wavefronts or more per CU stays, two where a lane has 16 bytes of 16-bit elements and registers to spare: more
         // blocks have more shares to write and to add (bf16 16384 x 4096: 71.4 us with 256 blocks, 74.4 with 512; 65536 x 512: 44.4, 37.3).
         grid = std::min(ceilDiv(c.rows, teams), units * (shape.chunks * vec < 16 ? 2 : 1));
-        shares = parameters ? grid : 0;
+        if (parameters) a.sharesOfBlock = ceilDiv(ceilDiv(c.rows, teams * grid), kRowsOfShare);
+        shares = parameters ? grid * a.sharesOfBlock : 0;
     } else if (parameters) {
         columnsKernel = c.dtype == THORHIP_FP32 ? columnsOf<float>(codes) : c.dtype == THORHIP_FP16 ? columnsOf<f16>(codes) : columnsOf<bf16>(codes);
         columnsGrid.x = columnBlocksOf(shape);
-        columnsGrid.y = std::min(ceilDiv(c.rows, 256 / columnLanes(kManyChunks)), std::max(1u, 8 * units / columnsGrid.x));
+        constexpr uint32_t kGroups = 256 / columnLanes(kManyChunks);  // of rows at a time
+        columnsGrid.y = std::min(ceilDiv(c.rows, kGroups), std::max(1u, 8 * units / columnsGrid.x));
+        columnsGrid.y = std::min(std::max(columnsGrid.y, ceilDiv(c.rows, kGroups * kRowsOfShare)), 65535u);
         shares = columnsGrid.y > 1 ? columnsGrid.y : 0;
     }
     const size_t workspace = (size_t)shares * 2 * c.columns * sizeof(float);
