@@ -856,17 +856,18 @@ uint32_t forwardBlocks(Shape s, uint32_t columns, int vec, uint32_t threads, boo
     }
     return std::max(1u, (waves * 64 + threads / 2) / threads);
 }
-// The team of a backward row.  Blocks of 768 lanes have registers for fp32 rows from the input only where those are full or, in teams of
-// all 768, whole; other rows take the next power of two (13107 x 2560 66.9 us, with 192 lanes 85.5; 6553 x 5121 70.9 and 93.8; 3048 x
-// 11008 83.6 with 1024 lanes, 91.5 with 768, 72.2 as whole rows).
+// The team of a backward row.  Blocks of 768 lanes have registers for fp32 rows where those are full, from codes whole ones too, and in
+// teams of all 768 any whole ones; other rows take the next power of two (from the input 13107 x 2560 67.7 us, with 192 lanes 85.5; 6552 x
+// 5121 74.7 and 93.8; 3048 x 11008 83.6 with 1024 lanes, as whole rows of 768 73.8; forward and backward from codes 16360 x 2051 124.5 us,
+// with 192 lanes 132.2; 5462 x 6143 122.3 and 126.8; 3727 x 9001 137.0 and 141.4, but 8190 x 4097 127.9 and 126.7).
 Shape backwardShapeOf(uint32_t columns, int vec, bool codes) {
     const Shape s = shapeOf(columns, vec, false);
-    const bool room = codes || vec == 8 || s.lanes % 3 != 0 || isFull(s, columns, vec) || (s.lanes == 768 && isWhole(s, columns, vec));
+    const bool room = vec == 8 || s.lanes % 3 != 0 || isFull(s, columns, vec) || ((codes || s.lanes == 768) && isWhole(s, columns, vec));
     return room ? s : shapeOf(columns, vec, true);
 }
 template <typename T, int LANES, bool CODES, Fit FIT>
 Backward backwardOfThree() {
-    constexpr bool ROOM = CODES || sizeof(T) == 2 || FIT == Fit::Full || (LANES == 768 && FIT == Fit::Whole);
+    constexpr bool ROOM = sizeof(T) == 2 || FIT == Fit::Full || ((CODES || LANES == 768) && FIT == Fit::Whole);
     if constexpr (ROOM) return layerNormBackward<T, LANES, 16 / kVec<T>, CODES, FIT>;
     return nullptr;
 }
