@@ -689,6 +689,10 @@ class ActivationCheckpoint:
     @staticmethod
     def allocate(dimensions: Sequence[int], dtype: DataType, gpu_num: int = 0) -> "ActivationCheckpoint":
         dims = [int(d) for d in dimensions]
+        if not dims:
+            raise ValueError("An activation checkpoint requires at least one axis.")
+        if dtype not in (DataType.fp8_e4m3, DataType.fp8_e5m2, DataType.int8):
+            raise ValueError(f"An activation checkpoint supports checkpoints in fp8_e4m3, fp8_e5m2 and int8, got {dtype!r}.")
         scales = dims[:-1] + [-(-dims[-1] // ActivationCheckpoint.BLOCK_ELEMENTS)]
         place = Placement(DeviceType.gpu, gpu_num)
         return ActivationCheckpoint(PhysicalTensor(place, PhysicalTensor.Descriptor(dtype, dims)),
