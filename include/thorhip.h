@@ -151,7 +151,7 @@ typedef struct thorhip_layer_norm {
     int checkpoint_dtype; /* 0: none */
     int extent_is_64;
     uint32_t rows, columns, inner_rows;
-    float epsilon;
+    float epsilon; /* positive, finite and normal */
     thorhip_rows input, output;
     const void* weight; /* [columns]; NULL: ones */
     const void* bias;   /* [columns]; NULL: zeros */

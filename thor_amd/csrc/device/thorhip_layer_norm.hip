@@ -14,6 +14,7 @@
 #include "thorhip_rows.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace {
@@ -969,6 +970,7 @@ int thorhip_layer_norm_forward(const thorhip_layer_norm* call, void* stream, int
     THORHIP_REQUIRE(c.checkpoint_dtype == 0 || knownFormat(c.checkpoint_dtype), "thorhip_layer_norm_forward: checkpoint dtype %d", c.checkpoint_dtype);
     THORHIP_REQUIRE(c.rows > 0 && c.columns > 0 && c.rows < (1u << 31) && c.columns < (1u << 24), "thorhip_layer_norm_forward: %u rows of %u columns", c.rows,
                     c.columns);
+    THORHIP_REQUIRE(c.epsilon > 0.0f && std::isnormal(c.epsilon), "thorhip_layer_norm_forward: epsilon %g", c.epsilon);
     THORHIP_REQUIRE(c.input.data != nullptr && c.output.data != nullptr && c.mean != nullptr && c.rstd != nullptr, "thorhip_layer_norm_forward: NULL tensor");
     THORHIP_REQUIRE(c.checkpoint_dtype == 0 || (c.codes != nullptr && c.scales != nullptr), "thorhip_layer_norm_forward: no checkpoint");
     ForwardArgs a{};
