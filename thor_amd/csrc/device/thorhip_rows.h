@@ -48,11 +48,12 @@ constexpr int kCheckpointBlock = 128;
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
-// What is known of a row when its kernel is compiled.  Any: nothing.  Whole: it ends with a whole chunk and has one; a lane without a
-// chunk of its own then works on the row's last chunk as that chunk's lane does, reading and writing the same bits, so that loads and
-// stores need no branches and the compiler can count what is on its way.  Blocks: the same of a row of whole blocks of codes, where the
-// lanes of a block work on the last block as its own lanes do, so that its codes and scale come out the same too.  Full: every lane has all
-// of its chunks.
+// What is known of a row when its kernel is compiled.  Any: nothing.  Whole: it ends with a whole chunk and has one, so there is no tail; a
+// lane without a chunk of its own can work on the row's last one as that chunk's lane does (source(), works()), reading and writing the
+// same bits, so that loads and stores need no branches and the compiler can count what is on its way.  The backward pass does; the forward
+// pass does not, where a block of codes would get another scale by it, and has the registers of the tail from it.  Blocks: a row of whole
+// blocks of codes, where the lanes of a block work on the last block as its own lanes do, so that its codes and scale come out the same
+// too; the forward pass does that.  Full: every lane has all of its chunks.
 enum class Fit { Any, Whole, Blocks, Full };
 
 // How a team of LANES lanes holds a row: whole chunks of VEC elements, chunk k of lane l at column (k * LANES + l) * VEC, and the
