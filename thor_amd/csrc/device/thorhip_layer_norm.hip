@@ -134,7 +134,7 @@ __device__ __forceinline__ void loadsArrived() { __builtin_amdgcn_s_waitcnt(0x0f
 
 // Rows of at most LANES * K chunks, a team of LANES lanes per row.  The blocks stay, keep weight and bias in registers and take every
 // gridDim-th row; a row is loaded while the one before it is worked on.
-// fp32 32768 x 1024 takes 45.4 us (5.9 TB/s), bf16 16384 x 4096 44.6 us (6.0 TB/s), bf16 8192 x 8192 with e4m3 codes 57.4 us (5.9 TB/s).
+// fp32 32768 x 1024 takes 43.7 us (6.1 TB/s), bf16 16384 x 4096 44.6 us (6.0 TB/s), bf16 8192 x 8192 with e4m3 codes 58.2 us (5.8 TB/s).
 template <typename T, int LANES, int K, bool CHECKPOINT, Fit FIT>
 __global__ __launch_bounds__(kForwardThreads<LANES>) void layerNormForward(ForwardArgs a) {
     constexpr int VEC = kVec<T>, TEAMS = kForwardThreads<LANES> / LANES;
@@ -238,7 +238,7 @@ struct LongSum {
 };
 
 // Rows of any length: a block of 1024 lanes per row, which reads it three times (the second and third time from the caches).  bf16
-// 4096 x 20000 takes 112 us (2.9 TB/s): a wavefront has a chunk on its way at a time, and folds between the readings.
+// 4096 x 20000 takes 112 us (2.9 TB/s), with e4m3 codes 189 us: a wavefront has a chunk on its way at a time, and folds between the readings.
 template <typename T, bool CHECKPOINT>
 __global__ __launch_bounds__(1024) void layerNormForwardLong(ForwardArgs a) {
     constexpr int VEC = kVec<T>, LANES = 1024;
@@ -386,7 +386,7 @@ __device__ __forceinline__ Elements<float> quarter(const float (&v)[K][VEC], int
 
 // Rows of at most LANES * K chunks, a team of LANES lanes per row.  The blocks stay and take every gridDim-th row; a row is loaded while
 // the one before it is worked on, where the lanes have the registers for both.
-// bf16 16384 x 4096 takes 68.4 us (6.0 TB/s with the shares), 8192 x 8192 from e4m3 codes 57.9 us (6.1 TB/s).
+// bf16 16384 x 4096 takes 69.6 us (5.9 TB/s with the shares), 8192 x 8192 from e4m3 codes 58.3 us (6.1 TB/s).
 template <typename T, int LANES, int K, bool CODES, Fit FIT>
 __global__ __launch_bounds__(kBackwardThreads<LANES>) void layerNormBackward(BackwardArgs a) {
     constexpr int VEC = kVec<T>, THREADS = kBackwardThreads<LANES>, TEAMS = THREADS / LANES;
