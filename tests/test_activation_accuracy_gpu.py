@@ -111,3 +111,19 @@ def test_gelu_in_fp32(stream, format):
     f, slope, _, _ = value_and_slope(GELU, x)
     within(dx, np.stack([slope, slope]), 12 * UNIT * terms(GELU, x) + LEAST, "slope")
     within(dz, f, 10 * UNIT * np.abs(f) + LEAST, "f backward")
+
+
+@pytest.mark.parametrize("kind", list(ph.ActivationKind), ids=lambda k: k.name)
+@pytest.mark.parametrize("dtype", [DataType.fp32, DataType.bf16], ids=lambda d: d.name)
+@pytest.mark.parametrize("format", FORMATS, ids=lambda f: f.name)
+def test_errors_times_multipliers_that_overflow(stream, format, dtype, kind):
+    """Where the slope is zero the gradient is, though error times multiplier is over fp32's range; where it is one, the gradient is too."""
+    cols = 261  # chunks and a tail
+    x = np.where(np.arange(cols) % 2 == 0, -200.0, 200.0)[None].repeat(2, 0)
+    save, gate = (ph.CheckpointSave(format).stamp(upload(v, DataType.fp32, stream)[0], stream) for v in (x, np.full((2, cols), 2.0**70)))
+    tdy, dy = upload(np.array([[2.0**70], [2.0**-70]]).repeat(cols, 1), dtype, stream)
+    plan = ph.CheckpointedActivationBackward(kind).stamp(tdy, save.get_checkpoint(), stream, multiplier_checkpoint=gate.get_checkpoint())
+    for p in (save, gate, plan):
+        p.run()
+    got = download(plan.get_input_gradient_tensor(), stream)
+    assert not got[:, ::2].any() and (got[0, 1::2] == np.inf).all() and np.abs(got[1, 1::2] - 1.0).max() <= rounding(1.0, dtype) + 6 * UNIT

@@ -331,7 +331,7 @@ __device__ __forceinline__ void backward(float dy, float& x, float& z) {
         x = finite<T>(x);
     } else {
         const Activated<T, KIND> f(x);
-        x = MULTIPLIED ? dy * z * f.slope() : dy * f.slope();
+        x = MULTIPLIED ? dy * (z * f.slope()) : dy * f.slope();  // a slope of zero before error times multiplier can overflow
         z = dy * f.finite();
     }
 }
@@ -340,7 +340,7 @@ __device__ __forceinline__ void backwardOfTable(const float* table, float dy, fl
     const float* entry = GeluTable<T, MULTIPLIED>::at(table, x);
     if constexpr (MULTIPLIED) {
         const float f = x * entry[1];
-        x = dy * z * entry[0];
+        x = dy * (z * entry[0]);
         z = dy * f;
     } else {
         x = dy * entry[0];
