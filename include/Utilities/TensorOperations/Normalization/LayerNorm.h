@@ -12,7 +12,8 @@
 // both); without them h is multiplied with ones and nothing is added.  mean and rstd are dense FP32 [..., 1].  The gradients of weight
 // and bias are dense [C] in the weight's type, FP32 without a weight.  All arithmetic is fp32, rounded once where a tensor is stored;
 // the output and the checkpoint have the precision of x - mean however large the mean is, the backward pass from the input that of the
-// stored mean.  Results are the same bits from run to run.  segment_offsets (UINT32 or UINT64 [B+1], read when the kernels run) marks a packed ragged
+// stored mean.  Differences of 2^64 and more have squares over fp32's range: rstd is zero then, and the output the bias.  Results are the
+// same bits from run to run.  segment_offsets (UINT32 or UINT64 [B+1], read when the kernels run) marks a packed ragged
 // batch: rows at and behind the last offset are neither read nor written and add nothing to a gradient.  No output may overlap another
 // tensor of the call.  Errors are std::invalid_argument.  The reference has no counterpart (its normalisations are a vendor library's).
 #pragma once
