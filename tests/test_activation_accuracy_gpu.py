@@ -127,3 +127,20 @@ def test_errors_times_multipliers_that_overflow(stream, format, dtype, kind):
         p.run()
     got = download(plan.get_input_gradient_tensor(), stream)
     assert not got[:, ::2].any() and (got[0, 1::2] == np.inf).all() and np.abs(got[1, 1::2] - 1.0).max() <= rounding(1.0, dtype) + 6 * UNIT
+
+
+@pytest.mark.parametrize("kind", [SWISH, GELU], ids=lambda k: k.name)
+def test_values_of_16_bits_near_ties(stream, kind):
+    """fp16 results below 2^-14 are multiples of 2^-24, and a value near a tie between two shows what it was before its rounding: within
+    the units that value_and_slope() counts, over twenty million products of an fp16 input and a multiplier that brings it there."""
+    x = np.arange(1 << 16, dtype=np.uint16).view(np.float16).astype(np.float32)
+    x = x[np.isfinite(x) & (np.abs(x) <= 2) & (np.abs(x) >= 2.0**-5)][None]
+    rows, cols = 1500, x.shape[1]
+    tx, x64 = upload(x, DataType.fp16, stream)
+    least = np.abs(value_and_slope(kind, x64)[0])
+    tz, z = upload(2.0**np.random.default_rng(0).uniform(-17, -14, (rows, cols)) / least, DataType.fp16, stream)
+    plan = ph.CheckpointedActivation(kind, DataType.int8).stamp(tx.alias_view([rows, cols], [0, 1]), stream, multiplier=tz)
+    plan.run()
+    f, _, f_off, _ = value_and_slope(kind, x64)
+    off = z * f_off + 2 * UNIT * np.abs(f * z)
+    within(download(plan.get_output_tensor(), stream), f * z, off + rounding(np.abs(f * z) + off, DataType.fp16), "f z")

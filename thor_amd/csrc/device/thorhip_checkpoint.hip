@@ -77,7 +77,7 @@ __device__ __forceinline__ Place placeOf(const CheckpointedArgs& a, u32 number) 
 // density, where the library's erfc has one of its own and a division.
 //
 // fp32: degree 9 (off by 3.5e-9), t from the sum 1 + 0.3 a as it is before its rounding.
-// 16 bits: degree 7 (off by 1.7e-7) at the hardware's reciprocal, some eight units of 2^-24, and H / 2^32 for bellTimes2To32().
+// 16 bits: degree 7 (off by 1.7e-7) at the hardware's reciprocal, some eight units of 2^-24, and H / 2^11 for bellTimes2To11().
 template <typename T>
 __device__ __forceinline__ float tailFactor(float a) {
     const float d = __builtin_fmaf(a, 0.3f, 1.0f);
@@ -97,7 +97,7 @@ __device__ __forceinline__ float tailFactor(float a) {
         p = __builtin_fmaf(p, t, 0.11968670040369034f);
         return p * t;
     }
-    constexpr float k = 0x1p-32f;
+    constexpr float k = 0x1p-11f;
     float p = 0.03542373867332211f * k;
     p = __builtin_fmaf(p, t, -0.1561584693838267f * k);
     p = __builtin_fmaf(p, t, 0.20455683389817478f * k);
@@ -109,13 +109,13 @@ __device__ __forceinline__ float tailFactor(float a) {
     return p * t;
 }
 
-// Results of 16 bits: 2^32 exp(-x^2 / 2) and 2^32 sigmoid(x), through the hardware's power of two and reciprocal.  Those know no numbers
-// below 2^-126, which a bf16 result can be made of: 2^32 brings everything that its type can hold into their range.  The exponents are
-// rounded to fp32, which costs x^2 or |x| units of 2^-24 in the tails, 1.2e-5 at most, and up to 7e-7 near zero; a result rounds by 2^-9
-// or 2^-12.
-__device__ __forceinline__ float bellTimes2To32(float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x * x, -0.72134752044448170f, 32.0f)); }
-__device__ __forceinline__ float sigmoidTimes2To32(float x) {
-    return __builtin_amdgcn_rcpf(0x1p-32f + __builtin_amdgcn_exp2f(__builtin_fmaf(x, -1.4426950408889634f, -32.0f)));
+// Results of 16 bits: 2^11 exp(-x^2 / 2) and 2^15 sigmoid(x), through the hardware's power of two and reciprocal.  Those know no numbers
+// below 2^-126, which a bf16 result can be made of: the factors bring everything that the types can hold into their range.  The exponents
+// are rounded to fp32, which costs x^2 or |x| units of 2^-24 in the tails, 1.2e-5 at most, and up to 3.4e-7 near zero, where larger
+// factors would cost more; a result rounds by 2^-9 or 2^-12.
+__device__ __forceinline__ float bellTimes2To11(float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x * x, -0.72134752044448170f, 11.0f)); }
+__device__ __forceinline__ float sigmoidTimes2To15(float x) {
+    return __builtin_amdgcn_rcpf(0x1p-15f + __builtin_amdgcn_exp2f(__builtin_fmaf(x, -1.4426950408889634f, -15.0f)));
 }
 
 // Results of fp32: a power of two as factor * 2^exponent, of an argument hi + lo with |lo| far below one, so that its rounding does not
@@ -163,7 +163,7 @@ struct Activated<T, THORHIP_RELU> {
 template <typename T>
 struct Activated<T, THORHIP_SWISH> {
     float x, s;
-    __device__ __forceinline__ explicit Activated(float x) : x(x), s(sigmoidTimes2To32(x) * 0x1p-32f) {}
+    __device__ __forceinline__ explicit Activated(float x) : x(x), s(sigmoidTimes2To15(x) * 0x1p-15f) {}
     __device__ __forceinline__ float finite() const { return any(); }
     __device__ __forceinline__ float any() const { return x * s; }
     __device__ __forceinline__ float slope() const { return __builtin_fmaf(any(), 1.0f - s, s); }
@@ -189,13 +189,13 @@ struct Activated<float, THORHIP_SWISH> {
 // here that the vector units bound); f' = exp(-x^2 / 2) (H(|x|) - |x| / sqrt(2 pi)) below zero, and that from one above.
 template <typename T>
 struct Activated<T, THORHIP_GELU> {
-    float x, h, e;  // h / 2^32, 2^32 e
-    __device__ __forceinline__ explicit Activated(float x) : x(x), h(tailFactor<T>(__builtin_fabsf(x))), e(bellTimes2To32(x)) {}
+    float x, h, e;  // h / 2^11, 2^11 e
+    __device__ __forceinline__ explicit Activated(float x) : x(x), h(tailFactor<T>(__builtin_fabsf(x))), e(bellTimes2To11(x)) {}
     __device__ __forceinline__ float finite() const { return __builtin_fmaf(-__builtin_fabsf(x), h * e, __builtin_fmaxf(x, 0.0f)); }
     __device__ __forceinline__ float any() const { return x * phi(); }
     __device__ __forceinline__ float phi() const { return x < 0.0f ? h * e : 1.0f - h * e; }
     __device__ __forceinline__ float slope() const {
-        const float below = e * __builtin_fmaf(__builtin_fabsf(x), -0.39894228040143268f * 0x1p-32f, h);
+        const float below = e * __builtin_fmaf(__builtin_fabsf(x), -0.39894228040143268f * 0x1p-11f, h);
         return x < 0.0f ? below : 1.0f - below;
     }
 };
